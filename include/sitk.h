@@ -611,7 +611,7 @@ int sitk_rope_axes(const sitk_rope_tensor* t, int count, const void* pos, int po
  *           both 16-byte aligned, sitk_act8_code_bytes / _step_bytes long
  * sitk_act8_gelu_fwd: g = gelu_erf(u) and u in 8 bits; sitk_act8_gelu_bwd: du = dg * gelu_erf'(u8).
  * sitk_act8_wgrad: dw[n][k] (+)= sum_m dy[m][n] x8[m][k], db[n] (+)= sum_m dy[m][n] (db may be NULL), f32; accumulate == 0 writes.
- *   dy (M, N) `dtype`; ws: sitk_act8_wgrad_ws_bytes of scratch (0: may be NULL).  Sums in a fixed order: two calls give the same
+ *   dy (M, N) `dtype`; M == 0: zeros, or nothing to add (dy, codes, steps may be NULL); ws: sitk_act8_wgrad_ws_bytes of scratch (0: may be NULL).  Sums in a fixed order: two calls give the same
  *   bits.  leading dimensions in elements.                                                           */
 size_t sitk_act8_code_bytes(int64_t rows, int cols);
 size_t sitk_act8_step_bytes(int64_t rows, int cols);

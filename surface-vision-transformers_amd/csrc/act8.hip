@@ -560,6 +560,14 @@ extern "C" int sitk_act8_wgrad(const void* dy, int64_t lddy, const int8_t* codes
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const size_t need = sitk_act8_wgrad_ws_bytes(M, N, K, dtype);
   SITK_REQUIRE(ws_bytes >= need && (ws || need == 0), "act8_wgrad: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  if (M == 0) {                                              // no product kernel, which would look for a first row: a join of no parts
+    if (accumulate) return SITK_OK;
+    const int64_t blocks = cdiv64((int64_t)N * K + N, 256);
+    hipLaunchKernelGGL(sitk::act8_join_kernel<1>, dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, s, (const float*)nullptr, dw, db,
+                       (int64_t)N, K, lddw, 0, 0);
+    SITK_LAUNCH_CHECK("act8_wgrad join");
+    return SITK_OK;
+  }
   const int vec = a8_vec(dy, lddy, dtype == SITK_F32 ? 4 : 2, dtype == SITK_F32 ? 4 : 8);
   const sitk::A8Plan plan = sitk::act8_plan(M, N, K, dtype, vec);
   sitk::A8Wgrad p{};

@@ -150,3 +150,20 @@ def test_wgrad_strides_and_no_rows(ops):
     assert float((e[0].double() - want).abs().max()) <= 108 * 2.0 ** -24 * float((wide[:1, :24].double().abs().t() * value_ref(x).abs().sum(0)).max())
     dW, db = ops.act8_wgrad(torch.empty(0, 24, device=DEV), ops.act8_pack(torch.empty(0, 40, device=DEV)))
     assert dW.shape == (24, 40) and float(dW.abs().max()) == 0.0 and float(db.abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N", [24, 21])
+def test_wgrad_without_rows(ops, dtype, N):
+    """Zeros in every element, rows of a wider buffer left as they are; added to a gradient: that gradient, bit for bit."""
+    p = ops.act8_pack(torch.empty(0, 40, device=DEV, dtype=TD[dtype]))
+    dy = torch.empty(0, N, device=DEV, dtype=TD[dtype])
+    junk = [torch.full((N, 40), math.nan, device=DEV) for _ in range(8)]       # what the allocator hands out next
+    del junk
+    dW, db = ops.act8_wgrad(dy, p)
+    assert dW.shape == (N, 40) and not dW.any() and db.shape == (N,) and not db.any()
+    wide = torch.randn(N, 43, device=DEV)
+    was, b = wide.clone(), torch.randn(N, device=DEV)
+    b_was = b.clone()
+    ops.act8_wgrad(dy, p, dW=wide[:, 1:41], db=b)
+    assert torch.equal(wide, was) and torch.equal(b, b_was)

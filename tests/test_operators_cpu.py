@@ -176,3 +176,15 @@ def test_block_c_refusals(sitk_mods):
     assert L.sitk_block_attention_bwd(desc(), 16, byref(rows), 16, 16, 16, 16, need - 1, 1, None) == -1
     assert L.sitk_block_attention_bwd(desc(), 16, byref(rows), 16, None, 16, 16, need, 1, None) == -1
     assert L.sitk_block_attention_bwd(desc(), 8, byref(rows), 16, 16, 16, 16, need, 1, None) == -1
+
+
+def test_act8_wgrad_without_rows(sitk_mods):
+    """No rows, null operands as empty tensors have them: added to what is there nothing is launched, else only the join that writes the
+    zeros (its launch fails here by name, where no device is)."""
+    _, rt = sitk_mods
+    for dtype in (0, 1, 2):
+        for N in (24, 21):                                      # rows of whole 16-byte chunks and others
+            assert rt.lib.sitk_act8_wgrad(None, N, None, None, 16, 40, 16, 0, N, 40, 1, None, 0, dtype, None) == 0, (dtype, N)
+            if not torch.cuda.is_available():
+                assert rt.lib.sitk_act8_wgrad(None, N, None, None, 16, 40, 16, 0, N, 40, 0, None, 0, dtype, None) == -2
+                assert b"join" in rt.lib.sitk_last_error()
