@@ -358,9 +358,11 @@ __global__ __launch_bounds__(256, NG > 6 ? 2 : 3) void block_select_kernel(const
     lo = -xor_max4(-lo);
     hi = xor_max4(hi);
     sum = xor_sum4(sum);
-    const bool odd = !(fabsf(sum) < 1e38f) || !(hi < 3e38f) || !(lo > -3e38f);   // a NaN or an infinity among the scores
     // 2^-17 |q| |kbar| per score; half planes end at 2^-24 (subnormal): 2^-25 sum |q| <= 2^-22 |q| more
     const float bound = qn * (kn * 0x1p-17f + (SITK_H16 == SITK_F16 ? 0x1p-22f : 0.f));
+    // A NaN or an infinity among the scores, or no bound for them (squares of finite |q| or |kbar| above 1.8e19 are not finite): all blocks
+    // again.  Below 1e37 it keeps `below` above the -infinity of blocks without a valid key, which are no candidates then.
+    const bool odd = !(fabsf(sum) < 1e38f) || !(hi < 3e38f) || !(lo > -3e38f) || !(bound < 1e37f);
     bool found = alive <= top_k, done = found || odd || r >= s.R;
     thr = -INFINITY;
     int reached = top_k;                                     // scores at or above thr
