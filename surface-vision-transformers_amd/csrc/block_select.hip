@@ -360,9 +360,12 @@ __global__ __launch_bounds__(256, NG > 6 ? 2 : 3) void block_select_kernel(const
     sum = xor_sum4(sum);
     // 2^-17 |q| |kbar| per score; half planes end at 2^-24 (subnormal): 2^-25 sum |q| <= 2^-22 |q| more
     const float bound = qn * (kn * 0x1p-17f + (SITK_H16 == SITK_F16 ? 0x1p-22f : 0.f));
-    // A NaN or an infinity among the scores, or no bound for them (squares of finite |q| or |kbar| above 1.8e19 are not finite): all blocks
-    // again.  Below 1e37 it keeps `below` above the -infinity of blocks without a valid key, which are no candidates then.
-    const bool odd = !(fabsf(sum) < 1e38f) || !(hi < 3e38f) || !(lo > -3e38f) || !(bound < 1e37f);
+    // A NaN or an infinity among the scores, or no bound for them: all blocks again.  The bound needs squares and products inside the range of
+    // 32 bits.  Squares of finite |q| or |kbar| above 1.8e19 are not; below 1e37 it keeps `below` above the -infinity of blocks without a
+    // valid key, which are no candidates then.  Small ones underflow: from norms of 2^-60 and a bound of 2^-100 on, what flushed planes (2^-126
+    // each), products and squares lose is far inside the bound.  So near > 0 wherever a score is not, and no more than top_k are sure.
+    const bool odd = !(fabsf(sum) < 1e38f) || !(hi < 3e38f) || !(lo > -3e38f) || !(bound < 1e37f) || !(bound > 0x1p-100f) ||
+                     !(fminf(qn, kn) > 0x1p-60f);
     bool found = alive <= top_k, done = found || odd || r >= s.R;
     thr = -INFINITY;
     int reached = top_k;                                     // scores at or above thr
