@@ -5,7 +5,7 @@
 
 namespace sitk {
 
-constexpr int BLK_MAX_NB = 2048;       // blocks of one sequence (the select kernel holds a row's scores in registers)
+constexpr int BLK_MAX_NB = 2048;       // blocks of one sequence (select: 16 rows' scores in a wave's registers up to 640, above them row by row in 64 bits)
 constexpr int BLK_MAX_TILES = 4096;    // 64-key tiles of one sequence (the attention kernels list a row tile's key tiles in LDS)
 
 struct BlkShape {
