@@ -48,6 +48,10 @@ class Attention(nn.Module):
         self.to_out = nn.Sequential(nn.Linear(inner, dim), nn.Dropout(dropout)) if self.project_out else nn.Identity()
 
 
+def _capturing(device):
+    return torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class FeedForward(nn.Module):
     def __init__(self, dim, hidden_dim, dropout):
         super().__init__()
@@ -67,7 +71,7 @@ class Transformer(nn.Module):
       * act8: training keeps the inputs of the linear layers and of GELU in 8 bits (about 29 D instead of 48 D bytes per token and layer
         in the 16-bit modes with mlp_dim = 4 D); forward values are unchanged."""
 
-    rotary, key_blocks, act8, _positions = None, None, False, None      # also of modules pickled before the options were there
+    rotary, key_blocks, act8, _positions, _positions_captured = None, None, False, None, ()     # also of modules pickled before the options were there
 
     def __init__(self, dim, depth, heads, dim_head, mlp_dim, dropout=0.0, compute_dtype="bf16", rotary=None, rotary_base=10000.0,
                  key_blocks=None, act8=False):
@@ -112,7 +116,8 @@ class Transformer(nn.Module):
         return not (self.training and self.p_dropout > 0) and (a is None or (a.dim_head == 64 and a.project_out))
 
     def set_positions(self, positions):
-        """Positions of the tokens for `rotary`: (N, axes), floating point or integers, one row per token (a class token included)."""
+        """Positions of the tokens for `rotary`: (N, axes), floating point or integers, one row per token (a class token included).  A captured
+        graph keeps the positions that it was captured with."""
         if self.rotary is None:
             raise SitkError("set_positions: the model has no rotary positions (rotary=None)")
         positions = torch.as_tensor(positions).detach()
@@ -127,10 +132,15 @@ class Transformer(nn.Module):
             raise SitkError("rotary positions are not set (SiT.set_patch_positions / Transformer.set_positions)")
         if self._positions.shape[0] != N:
             raise SitkError(f"rotary positions of {self._positions.shape[0]} tokens, the input has {N}")
-        key = str(device)
+        key, capturing = str(device), _capturing(device)
         if key not in self._positions_dev:
+            if capturing:
+                raise SitkError(f"rotary positions are not on {device} yet: run the model once before capturing it")
             self._positions_dev[key] = (self._positions.to(device), ops.rope_freqs(self.rotary, self.rotary_base, device))
-        return self._positions_dev[key]
+        inputs = self._positions_dev[key]
+        if capturing and not any(inputs is kept for kept in self._positions_captured):
+            self._positions_captured = (*self._positions_captured, inputs)     # a replay reads them, whatever set_positions has put in their place
+        return inputs
 
     def _attend(self, qkv, B, N, H, dh, scale):
         """(B, N, 3 H dh) -> (B, N, H dh): rotary positions, then attention over selected blocks or over all tokens."""

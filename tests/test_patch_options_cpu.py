@@ -55,3 +55,30 @@ def test_defaults_and_state_dict_are_unchanged(mods):
     assert set(plain.state_dict()) == set(full.state_dict())
     for opt in (dict(rotary=(4,)), dict(key_blocks=(64, 1)), dict(act8=True)):
         assert not sit.SiT(**KW, **opt).transformer.fused_ok()
+
+
+def test_positions_of_a_captured_graph_stay(mods, monkeypatch):
+    """Whatever a forward pass took under capture lives as long as the model (a replay reads it), also behind set_positions; passes outside a
+    capture keep nothing, and positions that are not on the device cannot be brought there under capture."""
+    import weakref
+    sit, SitkError = mods
+    t = sit.SiT(**KW, rotary=(4, 4, 4)).transformer
+    t.set_positions(torch.randn(11, 3))
+    monkeypatch.setattr(sit, "_capturing", lambda device: True)
+    with pytest.raises(SitkError, match="before capturing"):
+        t._rotary_inputs(11, "cpu")
+    seen = []
+    for capturing in (False, True, True, False):
+        t.set_positions(torch.randn(11, 3))
+        monkeypatch.setattr(sit, "_capturing", lambda device: False)
+        t._rotary_inputs(11, "cpu")
+        monkeypatch.setattr(sit, "_capturing", lambda device, c=capturing: c)
+        for _ in range(2):                                       # two layers
+            pos, freqs = t._rotary_inputs(11, "cpu")
+        seen.append((weakref.ref(freqs), pos.data_ptr(), pos.clone()))
+        del pos, freqs
+    t.set_positions(torch.randn(11, 3))
+    assert [ref() is not None for ref, _, _ in seen] == [False, True, True, False]
+    assert len(t._positions_captured) == 2
+    for (pos, freqs), (ref, ptr, was) in zip(t._positions_captured, seen[1:3]):
+        assert freqs is ref() and pos.data_ptr() == ptr and torch.equal(pos, was)

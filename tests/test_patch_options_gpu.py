@@ -400,3 +400,29 @@ def test_captured_training_step(mods):
         assert torch.equal(out, want)
         for (k, p), q in zip(m.named_parameters(), other.parameters()):
             assert float((p.grad - q.grad).norm()) <= 1e-5 * float(q.grad.norm()) + 1e-12, (i, k)
+
+
+def test_new_positions_leave_a_captured_graph_alone(mods):
+    """A graph of the forward pass, replayed behind set_positions and other allocations: the outputs of the positions it was captured with;
+    an eager pass takes the new ones, and a pass under capture that would have to bring them to the device is refused."""
+    sit, _, _, _ = mods
+    m, img, _ = build(sit, "bf16", rotary=(10, 10, 12), key_blocks=(64, 2))
+    x = img.clone()
+    with torch.no_grad():
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            want = m(x)
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = m(x)
+        new = m.transformer._positions.flip(0) * 1.5
+        m.transformer.set_positions(new)
+        junk = [torch.full((n,), 7.0, device=DEV) for n in range(1, 4000, 7)]
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            other = m(x)
+            assert not torch.equal(other, want) and len(junk)
