@@ -125,7 +125,8 @@ class Transformer(nn.Module):
             raise SitkError(f"set_positions: ({len(self.rotary)} axes) expected (tokens, {len(self.rotary)}), got {tuple(positions.shape)}")
         if positions.dtype not in (torch.float32, torch.float64, torch.int32, torch.int64):
             positions = positions.to(torch.float32 if positions.is_floating_point() else torch.int64)
-        self._positions, self._positions_dev = positions.cpu().clone(), {}
+        with torch.inference_mode(False):                        # kept beyond the call: a later training step saves them for its backward pass
+            self._positions, self._positions_dev = positions.cpu().clone(), {}
 
     def _rotary_inputs(self, N, device):
         if self._positions is None:
@@ -136,7 +137,8 @@ class Transformer(nn.Module):
         if key not in self._positions_dev:
             if capturing:
                 raise SitkError(f"rotary positions are not on {device} yet: run the model once before capturing it")
-            self._positions_dev[key] = (self._positions.to(device), ops.rope_freqs(self.rotary, self.rotary_base, device))
+            with torch.inference_mode(False):
+                self._positions_dev[key] = (self._positions.to(device), ops.rope_freqs(self.rotary, self.rotary_base, device))
         inputs = self._positions_dev[key]
         if capturing and not any(inputs is kept for kept in self._positions_captured):
             self._positions_captured = (*self._positions_captured, inputs)     # a replay reads them, whatever set_positions has put in their place

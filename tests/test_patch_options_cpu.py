@@ -82,3 +82,18 @@ def test_positions_of_a_captured_graph_stay(mods, monkeypatch):
     assert len(t._positions_captured) == 2
     for (pos, freqs), (ref, ptr, was) in zip(t._positions_captured, seen[1:3]):
         assert freqs is ref() and pos.data_ptr() == ptr and torch.equal(pos, was)
+
+
+def test_positions_set_and_first_used_in_inference_mode_train_later(mods):
+    sit, _ = mods
+    for set_inside in (False, True):
+        t = sit.SiT(**KW, rotary=(4, 4, 4)).transformer
+        given = torch.randn(11, 3)
+        if not set_inside:
+            t.set_positions(given)
+        with torch.inference_mode():
+            if set_inside:
+                t.set_positions(given)
+            t._rotary_inputs(11, "cpu")
+        pos, freqs = t._rotary_inputs(11, "cpu")
+        assert not pos.is_inference() and not freqs.is_inference() and torch.equal(pos, given)

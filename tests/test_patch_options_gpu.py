@@ -426,3 +426,19 @@ def test_new_positions_leave_a_captured_graph_alone(mods):
             assert torch.equal(out, want)
             other = m(x)
             assert not torch.equal(other, want) and len(junk)
+
+
+def test_training_behind_a_first_pass_in_inference_mode(mods):
+    sit, _, _, _ = mods
+    opt = dict(rotary=(10, 10, 12), key_blocks=(64, 2), act8=True)
+    m, img, w = build(sit, "bf16", **opt)
+    other, _, _ = build(sit, "bf16", **opt)
+    other.load_state_dict(m.state_dict())
+    other.transformer.set_positions(m.transformer._positions)
+    with torch.inference_mode():
+        seen = m(img).clone()
+    for x in (m, other):
+        (x(img) * w).sum().backward()
+    assert torch.equal(seen, other(img).detach())
+    for (k, p), q in zip(m.named_parameters(), other.parameters()):
+        assert float((p.grad - q.grad).norm()) <= 1e-5 * float(q.grad.norm()) + 1e-12, k
