@@ -608,7 +608,7 @@ int sitk_rope_axes(const sitk_rope_tensor* t, int count, const void* pos, int po
  * the smallest k such that rint(max |x| / 2^k) <= 127, -126 <= k <= 121 (SITK_F16: -24 <= k <= 9); code = rint(x / 2^k), at most
  * 127 in magnitude (which binds above 127.5 2^121 = 3.39e38, SITK_F16 65280, only).  The value code * 2^k is exact in `dtype`.  A group that holds an infinity or a NaN reads back as NaN.
  *   codes   (rows, cols rounded up to 32) signed bytes (pad: 0);  steps (rows, cols / 32 rounded up) bytes k + 127 (255: NaN)
- *           both 16-byte aligned, sitk_act8_code_bytes / _step_bytes long
+ *           sitk_act8_code_bytes / _step_bytes long, codes 16-byte aligned
  * sitk_act8_gelu_fwd: g = gelu_erf(u) and u in 8 bits; sitk_act8_gelu_bwd: du = dg * gelu_erf'(u8).
  * sitk_act8_wgrad: dw[n][k] (+)= sum_m dy[m][n] x8[m][k], db[n] (+)= sum_m dy[m][n] (db may be NULL), f32; accumulate == 0 writes.
  *   dy (M, N) `dtype`; M == 0: zeros, or nothing to add (dy, codes, steps may be NULL); ws: sitk_act8_wgrad_ws_bytes of scratch (0: may be NULL).  Sums in a fixed order: two calls give the same
@@ -632,7 +632,7 @@ int sitk_act8_wgrad(const void* dy, int64_t lddy, const int8_t* codes, const uin
  * Heads of 64 features; H query heads share Hk key heads (H % Hk == 0, head h reads key head h * Hk / H).  Tensors (B, N, heads, 64),
  * features contiguous, base and strides multiples of 16 bytes.
  * 1. sitk_block_pool: block j = keys j * block .. of one sample (block a multiple of 64, at most 1024; at most 2048 blocks, 262144 keys).
- *      pool (sitk_block_pool_bytes, 256-byte aligned) = the mean of every block's valid keys, first thing in it: f32 (B, Hk, nb rounded up
+ *      pool (sitk_block_pool_bytes, 16-byte aligned) = the mean of every block's valid keys, first thing in it: f32 (B, Hk, nb rounded up
  *      to 64, 64); behind them what selection and attention need (norms, counts, valid-key bits).  key_mask (B, Nk) bytes, row stride
  *      mask_b, nonzero = valid; NULL: all.  Masked keys are never read.
  * 2. sitk_block_select: for every query the top_k blocks with the largest q . mean, ties to the lower block, blocks without a valid

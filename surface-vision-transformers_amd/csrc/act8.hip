@@ -467,6 +467,7 @@ extern "C" size_t sitk_act8_step_bytes(int64_t rows, int cols) {
   SITK_REQUIRE((dtype) == SITK_F32 || (dtype) == SITK_BF16 || (dtype) == SITK_F16, name ": unknown dtype %d", (dtype));      \
   SITK_REQUIRE((rows) * (int64_t)cdiv((cols), 32) * 4 < (int64_t)0xFFFFFF00, name ": %lld x %d: too large for one call",     \
                (long long)(rows), (cols))
+#define A8_CODES(name, codes) SITK_REQUIRE((uintptr_t)(codes) % 16 == 0, name ": codes are not 16-byte aligned")
 #define A8_LD(name, ld, cols) SITK_REQUIRE((ld) >= (cols), name ": leading dimension %lld < %d", (long long)(ld), (cols))
 // rows that can be read `n` elements at a time
 static inline int a8_vec(const void* p, int64_t ld, int es, int n = 4) { return (uintptr_t)p % (n * es) == 0 && ld % n == 0; }
@@ -486,6 +487,7 @@ extern "C" int sitk_act8_pack(const void* x, int64_t ldx, int8_t* codes, uint8_t
                               sitk_stream_t stream) {
   SITK_REQUIRE(x && codes && steps, "act8_pack: null pointer");
   A8_COMMON("act8_pack", rows, cols, dtype);
+  A8_CODES("act8_pack", codes);
   A8_LD("act8_pack", ldx, cols);
   if (rows == 0) return SITK_OK;
   SITK_FORWARD_F16(dtype, sitk_act8_pack, x, ldx, codes, steps, rows, cols, dtype, stream);
@@ -500,6 +502,7 @@ extern "C" int sitk_act8_gelu_fwd(const void* u, int64_t ldu, void* g, int64_t l
                                   int cols, int dtype, sitk_stream_t stream) {
   SITK_REQUIRE(u && g && codes && steps, "act8_gelu_fwd: null pointer");
   A8_COMMON("act8_gelu_fwd", rows, cols, dtype);
+  A8_CODES("act8_gelu_fwd", codes);
   A8_LD("act8_gelu_fwd", ldu, cols);
   A8_LD("act8_gelu_fwd", ldg, cols);
   if (rows == 0) return SITK_OK;
@@ -515,6 +518,7 @@ extern "C" int sitk_act8_unpack(const int8_t* codes, const uint8_t* steps, void*
                                 sitk_stream_t stream) {
   SITK_REQUIRE(y && codes && steps, "act8_unpack: null pointer");
   A8_COMMON("act8_unpack", rows, cols, dtype);
+  A8_CODES("act8_unpack", codes);
   A8_LD("act8_unpack", ldy, cols);
   if (rows == 0) return SITK_OK;
   SITK_FORWARD_F16(dtype, sitk_act8_unpack, codes, steps, y, ldy, rows, cols, dtype, stream);
@@ -529,6 +533,7 @@ extern "C" int sitk_act8_gelu_bwd(const void* dg, int64_t lddg, const int8_t* co
                                   int64_t rows, int cols, int dtype, sitk_stream_t stream) {
   SITK_REQUIRE(dg && du && codes && steps, "act8_gelu_bwd: null pointer");
   A8_COMMON("act8_gelu_bwd", rows, cols, dtype);
+  A8_CODES("act8_gelu_bwd", codes);
   A8_LD("act8_gelu_bwd", lddg, cols);
   A8_LD("act8_gelu_bwd", lddu, cols);
   if (rows == 0) return SITK_OK;

@@ -1002,7 +1002,7 @@ static int blk_parts(const BlkShape& s, int dtype) {
 static int blk_attn_args(const char* who, const sitk_block_attn* p, int dtype, sitk::BlkAttn& a) {
   SITK_REQUIRE(p, "%s: null pointer", who);
   SITK_TRY(sitk::blk_check(who, p->B, p->Nq, p->Nk, p->H, p->Hk, p->block, dtype));
-  SITK_REQUIRE(p->mask && p->pool && p->lse, "%s: null pointer", who);
+  SITK_REQUIRE(p->mask && p->pool && p->lse && (uintptr_t)p->pool % 16 == 0, "%s: null or unaligned pointer", who);
   SITK_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "%s: scale = %g", who, (double)p->scale);
   SITK_TRY(sitk::blk_rows(who, "q", p->q, p->qs, dtype));
   SITK_TRY(sitk::blk_rows(who, "k", p->k, p->ks, dtype));
@@ -1029,7 +1029,7 @@ extern "C" int sitk_block_attention_fwd(const sitk_block_attn* p, void* ws, size
   sitk::BlkAttn a{};
   SITK_TRY(blk_attn_args("block_attention_fwd", p, dtype, a));
   const size_t need = sitk_block_attention_fwd_ws_bytes(p->B, p->Nq, p->Nk, p->H, p->Hk, p->block, dtype);
-  SITK_REQUIRE(ws_bytes >= need && (ws || need == 0), "block_attention_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
+  SITK_REQUIRE(ws_bytes >= need && (need == 0 || (ws && (uintptr_t)ws % 16 == 0)), "block_attention_fwd: workspace of %zu bytes, %zu needed", ws_bytes, need);
   SITK_FORWARD_F16(dtype, sitk_block_attention_fwd, p, ws, ws_bytes, dtype, stream);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   a.out = p->o;

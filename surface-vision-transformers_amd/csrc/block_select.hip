@@ -569,7 +569,7 @@ extern "C" int sitk_block_select(const void* q, const sitk_block_rows* qs, const
                                  int Nk, int H, int Hk, int block, int top_k, int dtype, sitk_stream_t stream) {
   SITK_TRY(sitk::blk_check("block_select", B, Nq, Nk, H, Hk, block, dtype));
   SITK_REQUIRE(top_k >= 1, "block_select: top_k = %d", top_k);
-  SITK_REQUIRE(qs && pool && index && mask, "block_select: null pointer");
+  SITK_REQUIRE(qs && pool && index && mask && (uintptr_t)pool % 16 == 0, "block_select: null or unaligned pointer");
   SITK_TRY(sitk::blk_rows("block_select", "q", q, *qs, dtype));
   SITK_FORWARD_F16(dtype, sitk_block_select, q, qs, pool, index, mask, B, Nq, Nk, H, Hk, block, top_k, dtype, stream);
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);

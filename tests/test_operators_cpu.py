@@ -188,3 +188,19 @@ def test_act8_wgrad_without_rows(sitk_mods):
             if not torch.cuda.is_available():
                 assert rt.lib.sitk_act8_wgrad(None, N, None, None, 16, 40, 16, 0, N, 40, 0, None, 0, dtype, None) == -2
                 assert b"join" in rt.lib.sitk_last_error()
+
+
+def test_unaligned_pools_codes_and_workspaces_are_refused(sitk_mods):
+    """What include/sitk.h asks for: 16 bytes."""
+    _, rt = sitk_mods
+    L, rows = rt.lib, rt.BlockRows(0, 64, 64)
+    assert L.sitk_act8_pack(16, 32, 24, 16, 3, 32, 1, None) == -1 and b"aligned" in L.sitk_last_error()
+    assert L.sitk_act8_unpack(24, 16, 16, 32, 3, 32, 1, None) == -1
+    assert L.sitk_act8_gelu_fwd(16, 32, 16, 32, 24, 16, 3, 32, 1, None) == -1
+    assert L.sitk_act8_gelu_bwd(16, 32, 24, 16, 16, 32, 3, 32, 1, None) == -1
+    assert L.sitk_block_select(16, C.byref(rows), 24, 16, 16, 1, 10, 100, 4, 2, 64, 3, 1, None) == -1 and b"aligned" in L.sitk_last_error()
+    for pool, ws in ((24, 16), (16, 24)):
+        d = rt.BlockAttn(1, 10, 1000, 4, 2, 64, 0.125, 16, 16, 16, rows, rows, rows, 16, 16, 16, pool)
+        assert L.sitk_block_attention_fwd_ws_bytes(1, 10, 1000, 4, 2, 64, 1) > 0
+        assert L.sitk_block_attention_fwd(C.byref(d), ws, 1 << 30, 1, None) == -1, (pool, ws)
+        assert L.sitk_block_attention_bwd(C.byref(d), 16, C.byref(rows), 16, 16, 16, ws, 1 << 30, 1, None) == -1, (pool, ws)
