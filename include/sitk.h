@@ -634,7 +634,8 @@ int sitk_act8_wgrad(const void* dy, int64_t lddy, const int8_t* codes, const uin
  * 1. sitk_block_pool: block j = keys j * block .. of one sample (block a multiple of 64, at most 1024; at most 2048 blocks, 262144 keys).
  *      pool (sitk_block_pool_bytes, 16-byte aligned) = the mean of every block's valid keys, first thing in it: f32 (B, Hk, nb rounded up
  *      to 64, 64); behind them what selection and attention need (norms, counts, valid-key bits).  key_mask (B, Nk) bytes, row stride
- *      mask_b, nonzero = valid; NULL: all.  Masked keys are never read.
+ *      mask_b, nonzero = valid; NULL: all.  Masked keys must be readable like
+ *      the others; whatever they hold (NaN, infinities) stays out.
  * 2. sitk_block_select: for every query the top_k blocks with the largest q . mean, ties to the lower block, blocks without a valid
  *      key left out; exact (as if scored in 64 bits).  index (B, H, Nq, top_k) ascending, -1 behind the last; mask: the same as bits,
  *      sitk_block_mask_words words.  sitk_block_mask makes the bits from an index of the caller's own (entries outside [0, nb) select
