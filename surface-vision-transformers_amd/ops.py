@@ -586,16 +586,52 @@ def _rope_sections(sections):
     return len(sections), sum(sections), min(sections), (C.c_int * len(sections))(*sections)
 
 
+def _reaches_zero(at, terms, budget):
+    """Whether at + sum of stride * d is 0 for some integers d within [lo, hi]; terms (stride, lo, hi) by falling stride.  Strides that nest, as
+    those of slices do, leave two d to try at most; a search that outlasts its budget counts as yes."""
+    if not terms:
+        return at == 0
+    (step, lo, hi), rest = terms[0], terms[1:]
+    least, most = sum(t * n for t, n, _ in rest), sum(t * n for t, _, n in rest)
+    for d in range(max(lo, -((at + most) // step)), min(hi, (-at - least) // step) + 1):
+        budget[0] -= 1
+        if budget[0] < 0 or _reaches_zero(at + step * d, rest, budget):
+            return True
+    return False
+
+
+def _byte_terms(shape, stride, es):
+    """(stride, size) of a (B, N, heads, dh) layout with contiguous features in bytes, sizes of 1 left out; the features are one run."""
+    return [(stride[i] * es, shape[i]) for i in range(3) if shape[i] > 1] + [(1, shape[3] * es)]
+
+
+@functools.lru_cache(maxsize=256)
+def _layouts_meet(apart, es, shape_a, stride_a, shape_b, stride_b):
+    span = {}
+    for step, n in _byte_terms(shape_a, stride_a, es):
+        lo, hi = span.get(step, (0, 0))
+        span[step] = (lo - (n - 1), hi)
+    for step, n in _byte_terms(shape_b, stride_b, es):
+        lo, hi = span.get(step, (0, 0))
+        span[step] = (lo, hi + n - 1)
+    return _reaches_zero(apart, sorted(((t, *r) for t, r in span.items()), reverse=True), [1000])
+
+
 def _share_features(a, b):
-    """Whether two (B, N, heads, dh) tensors of the same strides, as slices of one tensor are, have elements in common."""
-    if a.stride() != b.stride() or a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
-        return a.data_ptr() == b.data_ptr()
-    if a.storage_offset() > b.storage_offset():
-        a, b = b, a
-    apart, step, dh = b.storage_offset() - a.storage_offset(), max(a.stride(2), 1), a.shape[3]
-    if apart >= (a.shape[2] - 1) * step + dh:                  # b begins behind a's last head
-        return False
-    return apart % step < dh or step - apart % step < dh
+    """Whether two (B, N, heads, dh) tensors with contiguous features have memory in common."""
+    return _layouts_meet(b.data_ptr() - a.data_ptr(), a.element_size(), a.shape, a.stride(), b.shape, b.stride())
+
+
+@functools.lru_cache(maxsize=256)
+def _layout_meets_itself(es, shape, stride):
+    terms = sorted(_byte_terms(shape, stride, es), reverse=True)
+    return any(_reaches_zero(0, [(step, 1, n - 1)] + [(t, 1 - m, m - 1) for t, m in terms[i + 1:]], [1000])
+               for i, (step, n) in enumerate(terms))
+
+
+def _meets_itself(x):
+    """Whether two places of a (B, N, heads, dh) tensor with contiguous features are one in memory."""
+    return _layout_meets_itself(x.element_size(), x.shape, x.stride())
 
 
 def rope_axes(q, k, positions, freqs, sections, interleaved=False, inverse=False, inplace=False):
@@ -623,7 +659,9 @@ def rope_axes(q, k, positions, freqs, sections, interleaved=False, inverse=False
             raise rt.SitkError("rope_axes: the features of a head must be contiguous")
         if inplace and x is not None and any(s == 0 and n != 1 for s, n in zip(x.stride(), x.shape)):
             raise rt.SitkError("rope_axes: inplace on a broadcast tensor")
-    if inplace and k is not None and _share_features(q, k):
+        if inplace and x is not None and x.numel() and _meets_itself(x):
+            raise rt.SitkError("rope_axes: inplace on a tensor whose rows overlap")
+    if inplace and k is not None and q.numel() and k.numel() and _share_features(q, k):
         raise rt.SitkError("rope_axes: inplace on q and k that share features")
     rt.require_one_device(q, k, positions, freqs)
     if positions.stride(-1) != 1 and A > 1:

@@ -204,3 +204,64 @@ def test_unaligned_pools_codes_and_workspaces_are_refused(sitk_mods):
         assert L.sitk_block_attention_fwd_ws_bytes(1, 10, 1000, 4, 2, 64, 1) > 0
         assert L.sitk_block_attention_fwd(C.byref(d), ws, 1 << 30, 1, None) == -1, (pool, ws)
         assert L.sitk_block_attention_bwd(C.byref(d), 16, C.byref(rows), 16, 16, 16, ws, 1 << 30, 1, None) == -1, (pool, ws)
+
+
+def test_rope_inplace_overlaps(sitk_mods):
+    """q and k that share memory are refused whatever they are slices of, a tensor that meets itself too; disjoint slices are not."""
+    ops, rt = sitk_mods
+    pos, f = torch.zeros(5, 2), ops.rope_freqs((4, 4), device="cpu")
+
+    def call(q, k):
+        return lambda: ops.rope_axes(q, k, pos, f, (4, 4), inplace=True)
+
+    tok, smp, major = torch.zeros(2, 6, 3, 16), torch.zeros(3, 5, 3, 16), torch.zeros(2, 3, 6, 16).transpose(1, 2)
+    wide = torch.zeros(2, 5, 64)
+    q3 = wide[..., :48].view(2, 5, 3, 16)
+    for q, k in ((tok[:, :5], tok[:, 1:]), (tok[:, 1:], tok[:, :5]), (smp[:2], smp[1:]), (major[:, :5], major[:, 1:]),   # a token, a sample apart
+                 (q3, wide[..., 40:56].unsqueeze(2)), (q3, wide[..., 40:56].view(2, 5, 1, 16))):
+        refused(rt, call(q, k), "share features")
+    for q in (torch.zeros(1000).as_strided((2, 5, 3, 16), (240, 48, 8, 1)), torch.zeros(1000).as_strided((2, 5, 3, 16), (144, 48, 16, 1)),
+              torch.zeros(1000).as_strided((2, 5, 2, 16), (8, 80, 16, 1))):
+        refused(rt, call(q, None), "rows overlap")
+    # the next token's first head is what a second head of k behind q's last one reaches
+    far = torch.zeros(700)
+    refused(rt, call(far.as_strided((2, 5, 3, 16), (320, 64, 16, 1)), far.as_strided((2, 5, 2, 16), (320, 64, 16, 1), 48)), "share features")
+    packed = torch.zeros(2, 5, 8, 16)
+    apart = [(packed[:, :, :4], packed[:, :, 4:6]), (packed[:, :, 4:6], packed[:, :, :4]), (packed[:, :, ::2], packed[:, :, 1::2]),
+             (torch.zeros(2, 5, 3, 16), torch.zeros(2, 5, 1, 16)), (packed.transpose(1, 2).contiguous().transpose(1, 2)[:, :, :4], packed[:, :, :1]),
+             (packed[:1], packed[1:]), (wide[..., :48].view(2, 5, 3, 16), wide[..., 48:].unsqueeze(2))]
+    twice = torch.zeros(2, 10, 3, 16)
+    apart += [(twice[:, 0::2], twice[:, 1::2]), (twice[:, :5], twice[:, 5:]), (packed[:, :, :4], None)]
+    for q, k in apart:
+        refused(rt, call(q, k), "must live on a ROCm/HIP device")
+    empty = torch.zeros(0, 5, 3, 16)
+    refused(rt, call(empty, empty), "must live on a ROCm/HIP device")
+
+
+def test_overlap_search_against_listing_every_byte(sitk_mods):
+    """Random strided boxes in a small buffer: the answer of the search is that of the sets of addresses."""
+    import random
+    ops, _ = sitk_mods
+    rng, buf, seen = random.Random(3), torch.zeros(400, dtype=torch.uint8), set()
+
+    def box():
+        while True:
+            shape = [rng.randint(1, 3) for _ in range(3)] + [rng.randint(1, 4)]
+            stride = [rng.choice([4, 5, 8, 12, 16, 24, 36, 48, 60]) for _ in range(3)] + [1]
+            last = sum((n - 1) * t for n, t in zip(shape, stride))
+            if last < 380:
+                return buf.as_strided(shape, stride, rng.randint(0, 399 - last))
+
+    def places(x):
+        at = torch.tensor(x.storage_offset())
+        for n, t in zip(x.shape, x.stride()):
+            at = at[..., None] + torch.arange(n) * t
+        return at.flatten().tolist()
+
+    for _ in range(3000):
+        a, b = box(), box()
+        pa, pb = places(a), places(b)
+        assert ops._share_features(a, b) == bool(set(pa) & set(pb)), (a.shape, a.stride(), b.shape, b.stride())
+        assert ops._meets_itself(a) == (len(set(pa)) < len(pa)), (a.shape, a.stride())
+        seen |= {(bool(set(pa) & set(pb)), len(set(pa)) < len(pa))}
+    assert len(seen) == 4
