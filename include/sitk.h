@@ -611,8 +611,8 @@ int sitk_rope_axes(const sitk_rope_tensor* t, int count, const void* pos, int po
  *           sitk_act8_code_bytes / _step_bytes long, codes 16-byte aligned
  * sitk_act8_gelu_fwd: g = gelu_erf(u) and u in 8 bits; sitk_act8_gelu_bwd: du = dg * gelu_erf'(u8).
  * sitk_act8_wgrad: dw[n][k] (+)= sum_m dy[m][n] x8[m][k], db[n] (+)= sum_m dy[m][n] (db may be NULL), f32; accumulate == 0 writes.
- *   dy (M, N) `dtype`; M == 0: zeros, or nothing to add (dy, codes, steps may be NULL); ws: sitk_act8_wgrad_ws_bytes of scratch (0: may be NULL).  Sums in a fixed order: two calls give the same
- *   bits.  leading dimensions in elements.                                                           */
+ *   dy (M, N) `dtype`; M == 0: zeros, or nothing to add (dy, codes, steps may be NULL); ws: sitk_act8_wgrad_ws_bytes of scratch (0: may
+ *   be NULL).  Sums in a fixed order: two calls give the same bits.  leading dimensions in elements.        */
 size_t sitk_act8_code_bytes(int64_t rows, int cols);
 size_t sitk_act8_step_bytes(int64_t rows, int cols);
 int sitk_act8_pack(const void* x, int64_t ldx, int8_t* codes, uint8_t* steps, int64_t rows, int cols, int dtype, sitk_stream_t stream);
@@ -637,13 +637,17 @@ int sitk_act8_wgrad(const void* dy, int64_t lddy, const int8_t* codes, const uin
  *      mask_b, nonzero = valid; NULL: all.  Masked keys must be readable like
  *      the others; whatever they hold (NaN, infinities) stays out.
  * 2. sitk_block_select: for every query the top_k blocks with the largest q . mean, ties to the lower block, blocks without a valid
- *      key left out; exact (as if scored in 64 bits).  index (B, H, Nq, top_k) ascending, -1 behind the last; mask: the same as bits,
+ *      key left out; exact (as if scored in 64 bits; above 640 blocks it does score in 64 bits, some 40 times slower: take larger blocks).  index (B, H, Nq, top_k) ascending, -1 behind the last; mask: the same as bits,
  *      sitk_block_mask_words words.  sitk_block_mask makes the bits from an index of the caller's own (entries outside [0, nb) select
  *      nothing, an entry twice counts once).
  * 3. sitk_block_attention_fwd: o = softmax(scale q k^T) v over the valid keys of the selected blocks, contiguous (B, Nq, H, 64); lse
  *      (B, H, Nq) f32 natural log.  A query without a key: o = 0, lse = -inf.  _bwd: dq, dk, dv contiguous like their tensors, from o,
  *      lse and d_o; keys that nobody reads get zero.  The selection has no gradient.  All sums in a fixed order.  ws: scratch of
- *      sitk_block_attention_{fwd,bwd}_ws_bytes.                                                               */
+ *      sitk_block_attention_{fwd,bwd}_ws_bytes, 16-byte aligned.
+ *      Precision: scores, softmax statistics and sums in 32 bits.  SITK_BF16, SITK_F16: probabilities and dS are rounded to `dtype` for the
+ *      second product, like the operands, so o, dq, dk, dv are 1.2 to 1.6 times (r.m.s.) as far from the exact result as their own rounding; dk
+ *      and dv of up to 512 query rows (Nq H / Hk) are as exact as it.  SITK_F16: backward probabilities below 2^-14 (rows of more than
+ *      some 16000 keys of like score) lose bits to half's smallest step 2^-24.  SITK_F32: 32 bits throughout.               */
 typedef struct {
   int64_t b, n, h; /* strides in elements: sample, token, head */
 } sitk_block_rows;

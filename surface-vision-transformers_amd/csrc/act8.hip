@@ -96,7 +96,8 @@ SITK_DEV void a8_decode(float (&v)[8], u32x2 codes, uint32_t step) {
 
 // Standard normal tail Q(a) = P(X > a), a >= 0, and the density e^(-a^2 / 2) it comes with: erfc as t (a1 + .. + a5 t^4) e^(-x^2) with
 // t = 1 / (1 + p x), x = a / sqrt(2) (Abramowitz and Stegun, 7.1.26: off by at most 1.5e-7, half of that in Q).  1 + erf(x) in 32 bits is
-// off by as much (6e-8), and costs two branches of a polynomial each, which a wave takes both.
+// off by as much (6e-8), and costs two branches of a polynomial each, which a wave takes both.  For f32 too: u comes from 8 bits here, off by up to
+// half a step, 2^-8 of the largest of its group, so the derivative's last bits are not what limits du.
 SITK_DEV float normal_tail(float a, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.23164190f, a, 1.f));        // p / sqrt(2)
   e = fast_exp2(-0.72134752f * a * a);
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void act8_wgrad_kernel(A8Wgrad p) {
 // The 16-bit kernel: 256 x 128 tiles of dW, four waves of 128 x 64 (128 accumulator registers: 12 transposed fragments are read for 32
 // matrix instructions, where 64 x 64 per wave reads 16 for 32), 32 rows a stage.  dY comes by LDS-DMA through three stages; the codes go
 // through registers a stage ahead, are decoded there (each byte once per 256 columns of dY) and written beside it.
-// Bound: matrix instructions and the reads that feed them.  40992 rows, 768 -> 2304: 177 us, 820 TFLOP/s (the 64 x 64 kernel 1000 us); 20480
+// Bound: matrix instructions and the reads that feed them.  40992 rows, 768 -> 2304: 175 us, 830 TFLOP/s (the 64 x 64 kernel 1000 us); 20480
 // rows, 612 -> 192: 21 us, its parts' sums leave through HBM (102 parts of 0.47 MB).
 constexpr int W8_ROWS = 32, W8_N = 256, W8_K = 128;
 constexpr int W8_Y = W8_ROWS * W8_N * 2, W8_X = W8_ROWS * W8_K * 2, W8_STAGES = 3;

@@ -15,9 +15,9 @@
 // row tile's keys over up to 16 workgroups and joins them in order.
 // What 64 rows visit over what one row selects: 1.3 at 32 x 1281 tokens, top 8 of 21 blocks; 2.3 at 5121, 12 of 81; 3.6 at 20481, 16 of 321 (a
 // wave's 16 rows 1.2, 1.8, 2.5) -- the price of tiles, paid on the query side only.  Smaller tiles would read K and V more often from L2;
-// 32 rows a wave, 128 a workgroup, leave two workgroups a CU (forward at 32 x 1281 tokens 107 us instead of 84).
-// Measured, bf16, 6 heads: 32 x 1281 forward 84 us, dQ 112, dK / dV 137 (useful work 380, 430 and 470 TFLOP/s); 2 x 20481 forward 292, dQ 430, dK / dV
-// 242 (220, 225, 530).  16 single queries over 20481 keys, 12 heads on 3, top 16 of 161 blocks of 128: 15 us + join 5.
+// 32 rows a wave, 128 a workgroup, leave two workgroups a CU (forward at 32 x 1281 tokens 107 us where this took 84).
+// Measured, bf16, 6 heads (means of 150 calls): 32 x 1281 forward 80 us, dQ 110, dK / dV 128 (useful work 400, 440 and 500 TFLOP/s); 2 x 20481 forward
+// 297, dQ 424, dK / dV 241 (215, 230, 530).  16 single queries over 20481 keys, 12 heads on 3, top 16 of 161 blocks of 128: 14 us + join 5.
 // Scores, maxima, sums and accumulators are 32 bits.  P and dS are rounded to the operands' 16 bits once, for the second product (it has no
 // 32-bit operands); the row sum l adds P before that rounding, so lse stays a 32-bit value.
 // f32 (the verification mode): one plain tiled kernel per direction.
@@ -32,6 +32,10 @@ namespace sitk {
 // rounding, which is rowsum(dO o) of the exact o less that of the rounded one, and hands the exact one on; and dK and dV are taken
 // from P and dS as sums of two 16-bit values: both then as exact as their own rounding, and dK of a row with one key is zero.
 // Backward of 32 x 321 tokens, 6 heads, bf16: 63 us without, 70 with; with 1000 rows the gradients are 1.4 times as far off without it.
+// The rule asks for the rows of the key head, not of a block: dQ's kernel hands delta on before anyone has counted who selected a block, and the exact
+// delta for any number of rows costs more than it gives (2 x 20481 tokens: backward 656 us, 821 with it, 877 with P and dS of two values
+// too).  So a block that few of more than 512 rows select has its gradients off like any other of that call: r.m.s. error over that of their own
+// rounding dk 1.5 to 1.6, dv 1.3 to 1.7 for 2 to 2000 rows of 2048 (a single row: up to 2.3), 1.0 within the rule.
 constexpr int BLK_FINE_ROWS = 512;
 constexpr int BLK_LIST = 384;        // key tiles of the short list: with it three workgroups' LDS fit a CU
 

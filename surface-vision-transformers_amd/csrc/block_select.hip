@@ -12,9 +12,10 @@
 // Layout: a wave owns 16 rows; matrix tile i gives lane l the scores of row l & 15 with blocks 16 i + 4 (l >> 4) + 0..3, so a row is spread
 // over four lanes and the whole search for its threshold (count the scores at or above a guess, move the guess between the two
 // nearest known counts by their logarithms) runs in registers for 16 rows at once.  The planes pass through LDS, 64 blocks at a time, for
-// the four waves of a workgroup.
-// Bound: vector issue (search and bits; the products are 20 us of the 157 at 2 x 20481 rows, 6 heads, 321 blocks, bf16); 32 x 1281 rows, 21 blocks:
-// 40 us.  pool: HBM; 32 x 1281 keys, 6 heads 13 us (2.4 TB/s), 16 x 20481 keys, 3 heads 25 us (5.0 TB/s).
+// the four waves of a workgroup.  Above 640 blocks (BLK_MAX_NB are allowed) the registers do not hold the scores and every row goes in 64 bits:
+// 81921 rows, 6 heads, 18.3 ms with 1281 blocks of 64 keys, 0.28 ms with 321 of 256 -- long sequences want larger blocks.
+// Bound: vector issue (search and bits; the products are 20 us of the 156 at 2 x 20481 rows, 6 heads, 321 blocks, bf16); 32 x 1281 rows, 21 blocks:
+// 39 us.  pool: HBM; 32 x 1281 keys, 6 heads 12 us (2.5 TB/s: a workgroup has one 8 KB block to load and join), 16 x 20481 keys, 3 heads 25 us (5.0 TB/s).
 #include "block_common.h"
 
 namespace sitk {

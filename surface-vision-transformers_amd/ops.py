@@ -897,7 +897,8 @@ def _selection(index, pool):
 
 
 def block_select(q, pool, top_k):
-    """The top_k blocks of `pool` with the largest q . mean key for every query of q (B, Nq, H, 64): a BlockSelection."""
+    """The top_k blocks of `pool` with the largest q . mean key for every query of q (B, Nq, H, 64): a BlockSelection.  Fast up to 640
+    blocks; more (at most 2048) are ranked row by row in 64 bits."""
     code = _io_code(q)
     top_k = int(top_k)
     if not (q.dim() == 4 and q.shape[3] == 64):
@@ -964,7 +965,7 @@ def _block_desc(q, k, v, o, lse, sel, scale):
 
 def block_attention_fwd(q, k, v, sel, scale):
     """softmax(scale q k^T) v over the valid keys of each query's blocks: (o (B, Nq, H, 64), lse (B, H, Nq) f32).  A query without a
-    key gets o = 0, lse = -inf."""
+    key gets o = 0, lse = -inf.  bf16, f16: the probabilities are rounded to 16 bits for the product with v (statistics and sums: 32)."""
     code, scale = _block_attn(q, k, v, sel, scale, "block_attention_fwd")
     rt.require_one_device(q, k, v, sel.mask)
     q, k, v = _heads64(q, "q"), _heads64(k, "k"), _heads64(v, "v")
@@ -982,7 +983,8 @@ def block_attention_fwd(q, k, v, sel, scale):
 
 
 def block_attention_bwd(q, k, v, o, d_o, lse, sel, scale):
-    """(dq, dk, dv) of block_attention_fwd; o and lse are what it returned for the same q, k, v, sel and scale."""
+    """(dq, dk, dv) of block_attention_fwd; o and lse are what it returned for the same q, k, v, sel and scale.  bf16, f16: probabilities and
+    score gradients are rounded to 16 bits for the second products, but for dk and dv of up to 512 query rows per key head."""
     code, scale = _block_attn(q, k, v, sel, scale, "block_attention_bwd")
     for x, n in ((o, "o"), (d_o, "d_o")):
         if not (x.shape == q.shape and x.dtype == q.dtype):
