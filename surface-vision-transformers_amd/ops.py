@@ -856,7 +856,7 @@ def _heads64(x, what):
     if s3 == 1 and not ((s0 | s1 | s2) & m) and s1 < 1 << 23 and not x.data_ptr() & 15:
         return x
     if s3 != 1 or x.data_ptr() & 15 or s1 >= 1 << 23 or any(x.stride(i) & m and x.shape[i] > 1 for i in range(3)):
-        return x.contiguous() if not x.is_contiguous() else x.clone()
+        return x.clone(memory_format=_DENSE)                     # (strides of sizes of 1 too, which contiguous() leaves as they are)
     return torch.as_strided(x, x.shape, [x.stride(i) if x.shape[i] > 1 else 0 for i in range(3)] + [1])
 
 

@@ -265,3 +265,19 @@ def test_overlap_search_against_listing_every_byte(sitk_mods):
         assert ops._meets_itself(a) == (len(set(pa)) < len(pa)), (a.shape, a.stride())
         seen |= {(bool(set(pa) & set(pb)), len(set(pa)) < len(pa))}
     assert len(seen) == 4
+
+
+def test_heads_as_the_kernels_read_them(sitk_mods):
+    """Any layout of q, k, v comes out with features side by side, base and strides of whole 16 bytes, and the same values; aligned ones as
+    they are."""
+    ops, _ = sitk_mods
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        for shape in ((1, 1, 1, 64), (2, 1, 1, 64), (1, 5, 1, 64), (1, 1, 3, 64), (2, 5, 3, 64)):
+            x = torch.randn(shape).to(dtype)
+            odd = torch.cat([x[..., :3], x], -1)[..., 3:]
+            for y in (x, odd, x.transpose(1, 2).contiguous().transpose(1, 2), x.transpose(2, 3).contiguous().transpose(2, 3),
+                      torch.cat([x, x[..., :1]], -1)[..., :64], x.flatten()[None, None, None, :64].expand(shape), odd[:, :1], odd[:1, :, :1]):
+                z = ops._heads64(y, "x")
+                m = 16 // z.element_size()
+                assert torch.equal(z, y) and z.stride(3) == 1 and z.data_ptr() % 16 == 0 and all(s % m == 0 for s in z.stride()[:3])
+            assert ops._heads64(x, "x") is x or any(s % 4 for s in x.stride()[:3])
