@@ -653,7 +653,7 @@ typedef struct {
 } sitk_block_rows;
 typedef struct {
   int B, Nq, Nk, H, Hk, block;
-  float scale; /* > 0 */
+  float scale; /* 2^-100 to 2^100 */
   const void *q, *k, *v;
   sitk_block_rows qs, ks, vs;
   void* o; /* written by _fwd, read by _bwd */

@@ -1007,7 +1007,8 @@ static int blk_attn_args(const char* who, const sitk_block_attn* p, int dtype, s
   SITK_REQUIRE(p, "%s: null pointer", who);
   SITK_TRY(sitk::blk_check(who, p->B, p->Nq, p->Nk, p->H, p->Hk, p->block, dtype));
   SITK_REQUIRE(p->mask && p->pool && p->lse && (uintptr_t)p->pool % 16 == 0, "%s: null or unaligned pointer", who);
-  SITK_REQUIRE(p->scale > 0.f && p->scale < INFINITY, "%s: scale = %g", who, (double)p->scale);
+  // lse / scale has to be a number (below 1e-37 it was not, and the gradients were zero)
+  SITK_REQUIRE(p->scale >= 0x1p-100f && p->scale <= 0x1p100f, "%s: scale = %g (2^-100 to 2^100)", who, (double)p->scale);
   SITK_TRY(sitk::blk_rows(who, "q", p->q, p->qs, dtype));
   SITK_TRY(sitk::blk_rows(who, "k", p->k, p->ks, dtype));
   SITK_TRY(sitk::blk_rows(who, "v", p->v, p->vs, dtype));

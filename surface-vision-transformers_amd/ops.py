@@ -951,8 +951,8 @@ def _block_attn(q, k, v, sel, scale, who):
         if x.shape != (pool.B, pool.Nk, pool.Hk, 64):
             raise rt.SitkError(f"{who}: {n} {tuple(x.shape)} does not belong to a selection over ({pool.B}, {pool.Nk}, {pool.Hk}, 64)")
     scale = float(scale)
-    if not (0.0 < scale < float("inf")):
-        raise rt.SitkError(f"{who}: scale = {scale}")
+    if not (2.0 ** -100 <= scale <= 2.0 ** 100):
+        raise rt.SitkError(f"{who}: scale = {scale} (2^-100 to 2^100)")
     return code, scale
 
 

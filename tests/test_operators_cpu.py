@@ -281,3 +281,18 @@ def test_heads_as_the_kernels_read_them(sitk_mods):
                 m = 16 // z.element_size()
                 assert torch.equal(z, y) and z.stride(3) == 1 and z.data_ptr() % 16 == 0 and all(s % m == 0 for s in z.stride()[:3])
             assert ops._heads64(x, "x") is x or any(s % 4 for s in x.stride()[:3])
+
+
+def test_scales_that_leave_32_bits_are_refused(sitk_mods):
+    ops, rt = sitk_mods
+    k, q, rows = torch.zeros(2, 300, 2, 64), torch.zeros(2, 10, 4, 64), rt.BlockRows(0, 64, 64)
+    pool = ops.BlockPool(torch.zeros(1 << 16, dtype=torch.uint8), 2, 300, 2, 64, torch.float32)
+    sel = ops.BlockSelection(torch.zeros(2, 4, 10, 3, dtype=torch.int32), torch.zeros(8, dtype=torch.int32), pool)
+    for scale in (1e-38, 1e-31, 2e30, 1e38):
+        refused(rt, lambda: ops.block_attention_fwd(q, k, k, sel, scale), "scale")
+        refused(rt, lambda: ops.block_attention_bwd(q, k, k, q, q, torch.zeros(2, 4, 10), sel, scale), "scale")
+        d = rt.BlockAttn(1, 10, 100, 4, 2, 64, scale, 16, 16, 16, rows, rows, rows, 16, 16, 16, 16)
+        assert rt.lib.sitk_block_attention_fwd(C.byref(d), 16, 1 << 30, 1, None) == -1 and b"scale" in rt.lib.sitk_last_error()
+        assert rt.lib.sitk_block_attention_bwd(C.byref(d), 16, C.byref(rows), 16, 16, 16, 16, 1 << 30, 1, None) == -1
+    for scale in (2.0 ** -100, 2.0 ** 100):
+        refused(rt, lambda: ops.block_attention_fwd(q, k, k, sel, scale), "must live on")
